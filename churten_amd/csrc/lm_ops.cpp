@@ -17,6 +17,7 @@
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -516,5 +517,13 @@ TORCH_LIBRARY_FRAGMENT(churten, m) {
 
 TORCH_LIBRARY_IMPL(churten, CUDA, m) { implement(m); }
 TORCH_LIBRARY_IMPL(churten, CPU, m) { implement(m); }
+
+// The gradients have no derivative of their own: asking for one raises (torch's
+// default for an operator of a library is a warning, and zeros).
+TORCH_LIBRARY_IMPL(churten, Autograd, m) {
+  m.impl("embedding_grad", torch::autograd::autogradNotImplementedFallback());
+  m.impl("qk_norm_rope_grad", torch::autograd::autogradNotImplementedFallback());
+  m.impl("distill_loss_grad", torch::autograd::autogradNotImplementedFallback());
+}
 
 }  // namespace churten

@@ -26,7 +26,8 @@ the indices i, t the replica's temperature and h its share of hard labels::
 ``distill_loss_grad`` (same arguments) returns the loss and the gradient of its
 sum over all rows in the logits, in one pass over them: a training step that
 has no other use of autograd's graph takes this one. ``distill_loss`` is
-differentiable in ``logits`` and composes with ``torch.func.vmap``.
+differentiable once in ``logits`` (a second derivative raises) and composes with
+``torch.func.vmap``.
 """
 
 from __future__ import annotations

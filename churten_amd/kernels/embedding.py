@@ -15,7 +15,8 @@
   another layer shares), where rows that no token names are not touched.
 
 All of them without the replica dimension are one replica's call. ``embedding``
-is differentiable in ``weight`` and composes with ``torch.func.vmap``.
+is differentiable in ``weight``, as often as asked for, and composes with
+``torch.func.vmap``; a derivative of ``embedding_grad`` itself raises.
 """
 
 from __future__ import annotations
@@ -59,9 +60,25 @@ def _setup(ctx, inputs, output):
 
 def _backward(ctx, grad):
     tokens, = ctx.saved_tensors
-    return embedding_grad(grad, tokens, ctx.num_embeddings, ctx.scale), None, None
+    # A compiled backward pass is not differentiated again.
+    once = torch.compiler.is_compiling() or (
+        _plain() and not (grad.requires_grad and torch.is_grad_enabled()))
+    form = embedding_grad if once else _grad_apply
+    return form(grad, tokens, ctx.num_embeddings, ctx.scale), None, None
 
 
+def _grad_setup(ctx, inputs, output):
+    _, tokens, _, ctx.scale = inputs
+    ctx.save_for_backward(tokens)
+
+
+def _grad_backward(ctx, grad):
+    # The gradient is linear in the incoming one; its transpose is the lookup.
+    tokens, = ctx.saved_tensors
+    return embedding(grad, tokens, ctx.scale), None, None, None
+
+
+_, _grad_apply, _ = differentiable("embedding_grad", _grad_setup, _grad_backward)
 _op, _apply, _plain = differentiable("embedding", _setup, _backward)
 
 

@@ -19,7 +19,8 @@ interleaved=False) -> (q, k)``
 anew from ``q`` and ``k``. Arithmetic is float32, each result rounded once.
 
 All tensors without the replica dimension are one replica's call. The operator
-is differentiable in q, k and the weights and composes with ``torch.func.vmap``.
+is differentiable once in q, k and the weights (a second derivative raises) and
+composes with ``torch.func.vmap``.
 """
 
 from __future__ import annotations

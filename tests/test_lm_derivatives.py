@@ -1,0 +1,108 @@
+"""Which derivatives the language-model operators have, and that asking for
+another one raises instead of giving zeros or nothing."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.func import grad as func_grad
+from torch.func import vmap
+
+from churten_amd import kernels as K
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+pytestmark = pytest.mark.parametrize("device", DEVICES)
+
+
+def table(device, replicas=True):
+    """A table of small whole numbers, whose sums and products are exact, and tokens."""
+    g = torch.Generator().manual_seed(1)
+    lead = (2,) if replicas else ()
+    weight = torch.randint(-3, 4, (*lead, 7, 5), generator=g).float()
+    return weight.to(device), torch.randint(0, 7, (*lead, 9), generator=g).to(device)
+
+
+def lookups(tokens):
+    """The operator and plain indexing, scaled by 2."""
+    at = (tokens,) if tokens.dim() == 1 else (torch.arange(2, device=tokens.device)[:, None],
+                                              tokens)
+    return lambda w: K.embedding(w, tokens, 2.0), lambda w: w[at] * 2.0
+
+
+def heads(device):
+    g = torch.Generator().manual_seed(2)
+    q, k = torch.randn(2, 3, 4, 8, generator=g), torch.randn(2, 3, 2, 8, generator=g)
+    w, angle = torch.randn(2, 8, generator=g), torch.randn(6, 4, generator=g)
+    positions = torch.randint(0, 6, (2, 3), generator=g)
+    return [t.to(device) for t in (q, k, w, w + 1, angle.cos(), angle.sin(), positions)]
+
+
+def rows(device):
+    g = torch.Generator().manual_seed(3)
+    row = [torch.randn(2, 3, 11, generator=g), torch.randn(2, 3, 4, generator=g),
+           torch.randint(0, 11, (2, 3, 4), generator=g), torch.tensor([1.0, 2.0])]
+    return [t.to(device) for t in row]
+
+
+def once_differentiable(device):
+    """(function of one tensor, that tensor) for each operator without a second derivative."""
+    _, *rest = heads(device)
+    _, *teacher = rows(device)
+    return [(lambda q: (K.qk_norm_rope(q, *rest)[0] ** 3).sum(), heads(device)[0]),
+            (lambda w: (K.qk_norm_rope(*heads(device)[:2], w, *rest[2:])[0] ** 3).sum(), rest[1]),
+            (lambda x: K.distill_loss(x, *teacher).sum(), rows(device)[0])]
+
+
+@pytest.mark.parametrize("replicas", [False, True])
+def test_embedding_is_differentiable_more_than_once(device, replicas):
+    weight, tokens = table(device, replicas)
+    ours, plain = lookups(tokens)
+
+    def penalty(lookup):  # every derivative up to the third is of use
+        def loss(w):
+            return (lookup(w) ** 4).sum()
+
+        leaf = weight.clone().requires_grad_()
+        first, = torch.autograd.grad(loss(leaf), leaf, create_graph=True)
+        second, = torch.autograd.grad((first ** 2).sum(), leaf, create_graph=True)
+        third, = torch.autograd.grad((loss(leaf) + second.sum()), leaf)
+        nested = func_grad(lambda w: (func_grad(loss)(w) ** 2).sum())(weight)
+        return first, second, third, nested
+
+    for got, want in zip(penalty(ours), penalty(plain)):
+        assert want.any() and torch.equal(got, want)
+
+
+def test_second_derivatives_of_embedding_under_vmap(device):
+    weight, tokens = table(device)
+
+    def curvature(w, ids):
+        return func_grad(lambda w: (func_grad(
+            lambda w: (K.embedding(w, ids, 2.0) ** 3).sum())(w) ** 2).sum())(w)
+
+    each = torch.stack([curvature(w, ids) for w, ids in zip(weight, tokens)])
+    assert each.any() and torch.equal(vmap(curvature)(weight, tokens), each)
+
+
+def test_a_second_derivative_that_is_not_there_raises(device):
+    for f, x in once_differentiable(device):
+        leaf = x.clone().requires_grad_()
+        first, = torch.autograd.grad(f(leaf), leaf, create_graph=True)
+        torch.testing.assert_close(first, func_grad(f)(x))  # the first is there
+        with pytest.raises(RuntimeError, match="not implemented"):
+            (f(leaf) + (first ** 2).sum()).backward()
+        with pytest.raises(RuntimeError, match="not implemented"):
+            func_grad(lambda x: (func_grad(f)(x) ** 2).sum())(x)
+
+
+def test_a_derivative_of_a_gradient_operator_raises(device):
+    _, tokens = table(device)
+    grad = torch.ones(2, 9, 5, device=device, requires_grad=True)
+    row = rows(device)
+    row[0].requires_grad_()
+    q, k, *rest = heads(device)
+    q.requires_grad_()
+    for out in (K.embedding_grad(grad, tokens, 7), K.distill_loss_grad(*row)[0],
+                K.qk_norm_rope_grad(torch.ones_like(q), torch.ones_like(k), q, k, *rest)[2]):
+        with pytest.raises(RuntimeError, match="not implemented"):
+            out.sum().backward()

@@ -5,8 +5,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.func import grad as func_grad
-from torch.func import vmap
+from torch.func import jvp, vmap
 
 from churten_amd import kernels as K
 
@@ -106,3 +107,25 @@ def test_a_derivative_of_a_gradient_operator_raises(device):
                 K.qk_norm_rope_grad(torch.ones_like(q), torch.ones_like(k), q, k, *rest)[2]):
         with pytest.raises(RuntimeError, match="not implemented"):
             out.sum().backward()
+
+
+def test_forward_mode_raises(device):
+    """A tangent that no derivative carries on is not dropped."""
+    weight, tokens = table(device)
+    row = rows(device)
+    q, k, *rest = heads(device)
+    calls = [(lambda w: K.embedding(w, tokens, 2.0), weight),
+             (lambda q: K.qk_norm_rope(q, k, *rest)[0], q),
+             (lambda w: K.qk_norm_rope(q, k, rest[0], w, *rest[2:])[1], rest[1]),
+             (lambda x: K.distill_loss(x, *row[1:]), row[0]),
+             (lambda t: K.distill_loss(*row[:3], t), row[3]),
+             (lambda g: K.embedding_grad(g, tokens, 7), weight[:, [0, 1, 2, 3, 4, 5, 6, 0, 1]]),
+             (lambda x: K.distill_loss_grad(x, *row[1:]), row[0])]
+    for call, x in calls:
+        with forward_ad.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward AD"):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward AD"):
+            jvp(call, (x,), (torch.ones_like(x),))
+        with forward_ad.dual_level():
+            call(x)  # no tangent: as ever

@@ -17,6 +17,7 @@
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -562,6 +563,50 @@ struct Underived<R(A...)> {
   static void add(torch::autograd::edge_list&, double) {}
 };
 
+// In place, as torch's own: a target that gradients would go through is refused or
+// remembers that they cannot, and its version counter rises.
+const auto& embedding_grad_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("churten::embedding_grad_", "")
+                             .typed<decltype(embedding_grad_)>();
+  return op;
+}
+
+void embedding_grad_underived(c10::DispatchKeySet keys, at::Tensor weight_grad,
+                              const at::Tensor& grad, const at::Tensor& tokens, double scale,
+                              bool accumulate) {
+  constexpr const char* op = "churten::embedding_grad_";
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(weight_grad) && !has_tangent(grad), op,
+                              " has no derivative in forward AD mode");
+  const bool any = at::GradMode::is_enabled() &&
+                   (needs_derivative(weight_grad) || needs_derivative(grad));
+  torch::autograd::check_inplace(weight_grad, any);
+  std::shared_ptr<torch::autograd::Node> node;
+  if (any) {
+    node = std::shared_ptr<torch::autograd::Node>(
+        new torch::autograd::NotImplemented(
+            op, torch::autograd::collect_next_edges(weight_grad, grad)),
+        torch::autograd::deleteNode);
+  }
+  {
+    const at::AutoDispatchBelowAutograd below;
+    embedding_grad_op().redispatch(keys & c10::after_autograd_keyset, weight_grad, grad, tokens,
+                                   scale, accumulate);
+  }
+  if (any) torch::autograd::rebase_history(weight_grad, node);
+}
+
+void embedding_grad_written(c10::DispatchKeySet keys, at::Tensor weight_grad,
+                            const at::Tensor& grad, const at::Tensor& tokens, double scale,
+                            bool accumulate) {
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    embedding_grad_op().redispatch(keys & c10::after_ADInplaceOrView_keyset, weight_grad, grad,
+                                   tokens, scale, accumulate);
+  }
+  torch::autograd::increment_version(weight_grad);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(churten, m) {
@@ -599,10 +644,15 @@ constexpr char kDistillLossGrad[] = "churten::distill_loss_grad";
 TORCH_LIBRARY_IMPL(churten, Autograd, m) {
   m.impl("embedding", &Underived<decltype(embedding)>::call<kEmbedding>);
   m.impl("embedding_grad", &Underived<decltype(embedding_grad)>::call<kEmbeddingGrad>);
+  m.impl("embedding_grad_", &embedding_grad_underived);
   m.impl("qk_norm_rope", &Underived<decltype(qk_norm_rope)>::call<kQkNormRope>);
   m.impl("qk_norm_rope_grad", &Underived<decltype(qk_norm_rope_grad)>::call<kQkNormRopeGrad>);
   m.impl("distill_loss", &Underived<decltype(distill_loss)>::call<kDistillLoss>);
   m.impl("distill_loss_grad", &Underived<decltype(distill_loss_grad)>::call<kDistillLossGrad>);
+}
+
+TORCH_LIBRARY_IMPL(churten, ADInplaceOrView, m) {
+  m.impl("embedding_grad_", &embedding_grad_written);
 }
 
 }  // namespace churten

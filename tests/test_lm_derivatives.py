@@ -129,3 +129,35 @@ def test_forward_mode_raises(device):
             jvp(call, (x,), (torch.ones_like(x),))
         with forward_ad.dual_level():
             call(x)  # no tangent: as ever
+
+
+def test_the_gradient_in_place_is_seen_by_autograd(device):
+    """As torch's own operators in place: the version counter rises, a saved tensor
+    that is overwritten is noticed, a leaf that requires gradients is refused."""
+    _, tokens = table(device)
+    grad = torch.ones(2, 9, 5, device=device)
+    flat = torch.zeros(2, 40, device=device)
+    out = flat[:, 1:36].view(2, 7, 5)
+    K.embedding_grad_(out, grad, tokens)
+    assert out._version == 1 and flat._version == 1
+    K.embedding_grad_(out, grad, tokens, 2.0, accumulate=True)
+    assert out._version == 2
+    leaf = torch.ones(2, 7, 5, device=device, requires_grad=True)
+    product = leaf * out
+    K.embedding_grad_(out, grad, tokens)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with pytest.raises(RuntimeError, match="leaf Variable that requires grad"):
+        K.embedding_grad_(leaf, grad, tokens)
+    assert (leaf == 1).all()
+    with torch.no_grad():
+        K.embedding_grad_(leaf, grad, tokens)  # as an optimizer writes to its parameters
+    assert torch.equal(leaf.detach(), K.embedding_grad(grad, tokens, 7))
+    # A target that gradients would go through: they would have to go through this.
+    target = leaf * 1
+    K.embedding_grad_(target, grad, tokens, accumulate=True)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        target.sum().backward()
+    with forward_ad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward AD"):
+            K.embedding_grad_(out, forward_ad.make_dual(grad, grad), tokens)

@@ -14,7 +14,8 @@ from __future__ import annotations
 
 import torch
 
-__all__ = ["OWN", "SHARED", "HYPER", "TABLE", "differentiable", "register_replica_vmap"]
+__all__ = ["OWN", "SHARED", "HYPER", "TABLE", "differentiable", "register_replica_vmap",
+           "without_derivative"]
 
 OWN = "own"  # every replica has one
 SHARED = "shared"  # the replicas may share one
@@ -92,3 +93,25 @@ def differentiable(name: str, setup, backward):
         return transforms() is None and not torch.compiler.is_compiling()
 
     return op, function.apply, plain
+
+
+class _WithoutDerivative(torch.autograd.Function):
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(t, what):
+        return t.view_as(t)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.what = inputs[1]
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError(f"derivative for {ctx.what} is not implemented")
+
+
+def without_derivative(t, what: str):
+    """``t`` for an operator whose backward pass forms no gradient of it: asking
+    for one raises instead of finding none."""
+    return _WithoutDerivative.apply(t, what) if t is not None and t.requires_grad else t

@@ -26,8 +26,8 @@ the indices i, t the replica's temperature and h its share of hard labels::
 ``distill_loss_grad`` (same arguments) returns the loss and the gradient of its
 sum over all rows in the logits, in one pass over them: a training step that
 has no other use of autograd's graph takes this one. ``distill_loss`` is
-differentiable once in ``logits`` (a second derivative raises) and composes with
-``torch.func.vmap``.
+differentiable once in ``logits`` and composes with ``torch.func.vmap``; asking for a
+second derivative, or for one in ``temperature``, ``weight`` or ``hard``, raises.
 """
 
 from __future__ import annotations
@@ -41,6 +41,7 @@ from churten_amd.kernels._replicas import (
     SHARED,
     differentiable,
     register_replica_vmap,
+    without_derivative,
 )
 
 distill_loss_grad = torch.ops.churten.distill_loss_grad
@@ -82,10 +83,14 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor,
                  weight: torch.Tensor | None = None, labels: torch.Tensor | None = None,
                  hard: torch.Tensor | None = None) -> torch.Tensor:
     """The rows' losses; see the module's description."""
-    call = _apply
+    if teacher_logits.requires_grad:
+        teacher_logits = teacher_logits.detach()
     if _plain() and not (logits.requires_grad and torch.is_grad_enabled()):
-        call = _op
-    return call(logits, teacher_logits, teacher_index, temperature, weight, labels, hard)
+        return _op(logits, teacher_logits, teacher_index, temperature, weight, labels, hard)
+    return _apply(logits, teacher_logits, teacher_index,
+                  without_derivative(temperature, "distill_loss in temperature"),
+                  without_derivative(weight, "distill_loss in weight"), labels,
+                  without_derivative(hard, "distill_loss in hard"))
 
 
 _INPUTS = [(OWN, 2), (SHARED, 2), (SHARED, 2), (HYPER, 0), (SHARED, 1), (SHARED, 1), (HYPER, 0)]

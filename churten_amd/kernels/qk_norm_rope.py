@@ -19,8 +19,8 @@ interleaved=False) -> (q, k)``
 anew from ``q`` and ``k``. Arithmetic is float32, each result rounded once.
 
 All tensors without the replica dimension are one replica's call. The operator
-is differentiable once in q, k and the weights (a second derivative raises) and
-composes with ``torch.func.vmap``.
+is differentiable once in q, k and the weights and composes with
+``torch.func.vmap``; asking for a second derivative, or for one in the angles, raises.
 """
 
 from __future__ import annotations
@@ -34,6 +34,7 @@ from churten_amd.kernels._replicas import (
     TABLE,
     differentiable,
     register_replica_vmap,
+    without_derivative,
 )
 
 qk_norm_rope_grad = torch.ops.churten.qk_norm_rope_grad
@@ -77,8 +78,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     """The normed and rotated ``(q, k)``; see the module's description."""
     tracked = (q.requires_grad or k.requires_grad or q_weight.requires_grad
                or k_weight.requires_grad) and torch.is_grad_enabled()
-    call = _op if _plain() and not tracked else _apply
-    return call(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if _plain() and not tracked:
+        return _op(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _apply(q, k, q_weight, k_weight, without_derivative(cos, "qk_norm_rope in cos"),
+                  without_derivative(sin, "qk_norm_rope in sin"), positions, eps, interleaved)
 
 
 _INPUTS = [(OWN, 3), (OWN, 3), (OWN, 1), (OWN, 1), (TABLE, 2), (TABLE, 2), (SHARED, 1)]

@@ -161,3 +161,48 @@ def test_the_gradient_in_place_is_seen_by_autograd(device):
     with forward_ad.dual_level():
         with pytest.raises((RuntimeError, NotImplementedError), match="forward AD"):
             K.embedding_grad_(out, forward_ad.make_dual(grad, grad), tokens)
+
+
+def test_an_input_without_a_derivative_does_not_lose_its_gradient_silently(device):
+    x, z, index, t = rows(device)
+    weight, share = torch.rand(2, 3, device=device), torch.rand(2, device=device)
+    labels = torch.randint(0, 11, (2, 3)).to(device)
+    q, k, qw, kw, cos, sin, positions = heads(device)
+    calls = [(lambda x, t: K.distill_loss(x, z, index, t), x, t),
+             (lambda x, w: K.distill_loss(x, z, index, t, w), x, weight),
+             (lambda x, h: K.distill_loss(x, z, index, t, weight, labels, h), x, share),
+             (lambda q, c: K.qk_norm_rope(q, k, qw, kw, c, sin, positions)[0], q, cos),
+             (lambda q, s: K.qk_norm_rope(q, k, qw, kw, cos, s, positions)[0], q, sin)]
+    for call, main, other in calls:
+        want, = torch.autograd.grad(call(leaf := main.clone().requires_grad_(), other).sum(), leaf)
+        for with_main in (False, True):
+            leaf = main.clone().requires_grad_(with_main)
+            learned = other.clone().requires_grad_()
+            out = call(leaf, learned)
+            with pytest.raises(RuntimeError, match="not implemented"):
+                out.sum().backward()
+            with pytest.raises(RuntimeError, match="not implemented"):
+                func_grad(lambda o: call(leaf.detach(), o).sum())(other)
+        # Where it is not asked for, the other gradient is there.
+        got, = torch.autograd.grad(call(leaf, learned).sum(), leaf)
+        assert torch.equal(got, want)
+        assert torch.equal(func_grad(lambda m: call(m, learned.detach()).sum())(main), want)
+        with torch.no_grad():
+            assert torch.equal(call(leaf, learned), call(main, other))
+        # A derivative in the one around a derivative in the other.
+        with pytest.raises(RuntimeError, match="not implemented"):
+            func_grad(lambda o: func_grad(lambda m: call(m, o).sum())(main).sum())(other)
+        each = vmap(func_grad(lambda m: call(m, learned.detach()).sum()))(torch.stack([main] * 2))
+        torch.testing.assert_close(each[1], want)
+
+
+def test_no_gradient_flows_to_the_teacher(device):
+    x, z, index, t = rows(device)
+    taught = z.clone().requires_grad_()
+    assert not K.distill_loss(x, taught, index, t).requires_grad
+    leaf = x.clone().requires_grad_()
+    K.distill_loss(leaf, taught, index, t).sum().backward()
+    assert taught.grad is None
+    assert torch.equal(leaf.grad, K.distill_loss_grad(x, z, index, t)[1])
+    both = func_grad(lambda x, z: K.distill_loss(x, z, index, t).sum(), argnums=(0, 1))(x, z)
+    assert torch.equal(both[0], leaf.grad) and not both[1].any()

@@ -235,7 +235,7 @@ __device__ __forceinline__ float add_entry(const Entry& entry, float x, float z_
   return e;
 }
 
-// The label of a row (-1: none) and the replica's share of it.
+// The label of a row (-1: none, or the replica has no share of it) and that share.
 struct Label {
   int64_t at = -1;
   float share = 0;
@@ -246,9 +246,15 @@ __device__ __forceinline__ Label label_of(const ts_distill_args& a, int64_t n, i
   if constexpr (HARD) {
     label.share = a.hard[n];
     label.at = index_at(a.labels, n, b);
-    if (label.at >= a.V) label.at = -1;
+    if (label.at >= a.V || label.share == 0) label.at = -1;
   }
   return label;
+}
+
+// A replica with nothing but hard labels has no teacher, whatever the entries hold.
+template <bool HARD>
+__device__ __forceinline__ void drop_unshared(float (&total)[5], const Label& label) {
+  if (HARD && label.share == 1) total[2] = 0;
 }
 
 // The loss from the totals: s, s1, Z, sum e (z - max z), sum e (x - m).
@@ -298,7 +304,8 @@ __device__ __forceinline__ float taken_at(int i, const int* index, const float* 
 template <bool HARD>
 __device__ __forceinline__ float taken_gradient(const Scales& k, float Z, float x, float taken,
                                                 bool labelled) {
-  float g = gradient<HARD>(k, x) - taken * (Z != 0 ? k.soft / Z : 0);
+  float g = gradient<HARD>(k, x);
+  if (Z != 0) g -= taken * (k.soft / Z);
   if (HARD && labelled) g -= k.hard;
   return g;
 }
@@ -379,6 +386,7 @@ __global__ __launch_bounds__(kMaxThreads) void row_kernel(Args args) {
   block_reduce<HARD ? 0 : 2>(total, shared.sums, Plus{}, 0.0f);
 
   const Label label = label_of<HARD>(a, n, b);
+  drop_unshared<HARD>(total, label);
   if (split == 0 && t == 0) {
     const float label_x = label.at >= 0 ? static_cast<float>(row.x[label.at]) : 0.0f;
     a.loss[row_at] = loss_of(total, tops[0], temperature, weight, label, label_x);
@@ -578,6 +586,7 @@ __global__ __launch_bounds__(kMaxThreads) void staged_kernel(Args args) {
   block_reduce<HARD ? 0 : 2>(total, shared.sums, Plus{}, 0.0f);
 #pragma unroll
   for (int i = 0; i < 5; ++i) total[i] = uniform(total[i]);
+  drop_unshared<HARD>(total, label);
   if (t == 0) a.loss[row_at] = loss_of(total, m, temperature, weight, label, label_x);
   const float Z = total[2];
   const bool zero = Z == 0 && label.at < 0;
@@ -596,7 +605,7 @@ __global__ __launch_bounds__(kMaxThreads) void staged_kernel(Args args) {
 
   // The entries' elements again: after the row's stores.
   __syncthreads();
-  if (entry.index >= 0) {
+  if (entry.index >= 0 && !zero) {
     const float taken = slots_log2 == 0 || shared.repeated != 0
                             ? taken_at(entry.index, index, e, K)
                             : own;

@@ -249,7 +249,8 @@ void distill_row(const ts_distill_args& a, int64_t n, int64_t b) {
   if (a.hard != nullptr) {
     share = a.hard[n];
     label = index_at(a.labels, n, b);
-    if (label >= a.V) label = -1;
+    // A part without a share is left out: it may be infinite.
+    if (label >= a.V || share == 0) label = -1;
   }
   float m = std::numeric_limits<float>::lowest();
   for (int64_t v = 0; v < a.V; ++v) m = std::fmax(m, static_cast<float>(x[v]));
@@ -270,7 +271,7 @@ void distill_row(const ts_distill_args& a, int64_t n, int64_t b) {
     own += e * d;
     cross += e * (static_cast<float>(x[i]) - m);
   }
-  const bool taught = Z != 0;
+  const bool taught = Z != 0 && share != 1;
   if (taught) {
     const float kl = (own - cross) / (Z * t) - std::log(Z) + static_cast<float>(std::log(s));
     loss += (1 - share) * t * t * kl;
@@ -295,7 +296,7 @@ void distill_row(const ts_distill_args& a, int64_t n, int64_t b) {
     for (int64_t k = 0; k < a.K; ++k) {
       if (entry(k) == v) taken += std::exp((z[k] - z_top) / t);
     }
-    return static_cast<T>(base(v) - taken * (taught ? soft / Z : 0) - (v == label ? hard : 0));
+    return static_cast<T>(base(v) - (taught ? taken * (soft / Z) : 0) - (v == label ? hard : 0));
   };
   for (int64_t k = 0; k < a.K; ++k) {
     if (entry(k) >= 0) grad[entry(k)] = corrected(entry(k));

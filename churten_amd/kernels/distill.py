@@ -21,7 +21,8 @@ the indices i, t the replica's temperature and h its share of hard labels::
 * ``weight`` ``(N, B)`` or ``(B,)``: a row of weight 0 (padding, a frozen replica)
   is not read, whatever its logits hold; its loss and gradient are 0.
 * ``labels`` ``(N, B)`` or ``(B,)``, given together with ``hard``: a label outside
-  ``[0, V)`` has no hard part.
+  ``[0, V)`` has no hard part. A replica with h = 0 has no hard part and one with
+  h = 1 none from the teacher, also where those would be infinite.
 
 ``distill_loss_grad`` (same arguments) returns the loss and the gradient of its
 sum over all rows in the logits, in one pass over them: a training step that

@@ -151,36 +151,46 @@ template <int VE, Pairing PAIRING>
 struct Turn {
   static constexpr int kAngles = PAIRING == kInside ? VE / 2 : VE;
   Vec<float, kAngles> cos, sin;
+  bool on;
 
   __device__ __forceinline__ void fetch(const QkArgs& s, bool turn, int64_t row, int at) {
-    cos = Vec<float, kAngles>(1.0f);
-    sin = Vec<float, kAngles>{};
-    if (turn && row >= 0) {
+    cos = sin = Vec<float, kAngles>{};
+    on = turn && row >= 0;
+    if (on) {
       cos = load<kAngles>(s.cos + row + at);
       sin = load<kAngles>(s.sin + row + at);
     }
   }
 };
 
-// Rotates the packs a, b by their angles, or back for SIGN = -1.
+template <int VE, int SIGN>
+__device__ __forceinline__ void rotate_inside(Vec<float, VE>& v, const Turn<VE, kInside>& t) {
+  if (t.on) {
+#pragma unroll
+    for (int i = 0; i < VE / 2; ++i) {
+      const float sin = t.sin[i] * SIGN, a = v[2 * i], b = v[2 * i + 1];
+      v[2 * i] = a * t.cos[i] - b * sin;
+      v[2 * i + 1] = b * t.cos[i] + a * sin;
+    }
+  }
+}
+
+// Rotates the packs a, b by their angles, or back for SIGN = -1. What does not
+// turn is left alone: turned by no angle, a x 1 - b x 0, an infinity would reach the
+// element beside it.
 template <int VE, Pairing PAIRING, int SIGN>
 __device__ __forceinline__ void rotate(Vec<float, VE>& a, Vec<float, VE>& b,
                                        const Turn<VE, PAIRING>& ta,
                                        const Turn<VE, PAIRING>& tb) {
   if constexpr (PAIRING == kAcross) {
-    const Vec<float, VE> sin = ta.sin * float(SIGN), x = a, y = b;
-    a = x * ta.cos - y * sin;
-    b = y * ta.cos + x * sin;
-  } else {
-#pragma unroll
-    for (int i = 0; i < VE / 2; ++i) {
-      const float sa = ta.sin[i] * SIGN, sb = tb.sin[i] * SIGN;
-      const float a0 = a[2 * i], a1 = a[2 * i + 1], b0 = b[2 * i], b1 = b[2 * i + 1];
-      a[2 * i] = a0 * ta.cos[i] - a1 * sa;
-      a[2 * i + 1] = a1 * ta.cos[i] + a0 * sa;
-      b[2 * i] = b0 * tb.cos[i] - b1 * sb;
-      b[2 * i + 1] = b1 * tb.cos[i] + b0 * sb;
+    if (ta.on) {
+      const Vec<float, VE> sin = ta.sin * float(SIGN), x = a, y = b;
+      a = x * ta.cos - y * sin;
+      b = y * ta.cos + x * sin;
     }
+  } else {
+    rotate_inside<VE, SIGN>(a, ta);
+    rotate_inside<VE, SIGN>(b, tb);
   }
 }
 

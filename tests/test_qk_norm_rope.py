@@ -246,3 +246,46 @@ def test_refusals(device):
         K.qk_norm_rope_grad(dq, dk[:, :, :1], q, k, qw, kw, cos, sin, positions)
     with pytest.raises(RuntimeError, match="grad_q must have dtype"):
         K.qk_norm_rope_grad(dq.half(), dk, q, k, qw, kw, cos, sin, positions)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,rot", [(64, 64), (64, 32), (128, 128), (96, 48), (80, 40), (48, 24),
+                                   (33, 16), (33, 0), (257, 128), (24, 8)])
+def test_infinities_stay_with_their_pair(device, D, rot, dtype, interleaved):
+    """An infinite element makes its head's norm infinite: it becomes NaN and the
+    head's other elements 0. NaN reaches another element by a rotation alone, not
+    beyond ``rot`` nor at a position outside the tables."""
+    N, M, H, P = 1, 2 * D, 3, 8
+    g = torch.Generator().manual_seed(13)
+    x = torch.randn(N, M, H, D, generator=g)
+    at = torch.arange(M) % D
+    x[0, torch.arange(M), 1, at] = torch.inf  # in one of the token's heads
+    positions = torch.where(torch.arange(M) < D, 3, P)  # the second half: outside
+    w = 1 + torch.rand(N, D, generator=g)
+    angle = 0.5 + torch.rand(P, rot // 2, generator=g)
+    args = [t.to(device) for t in (x.to(dtype), x[:, :, 1:].to(dtype).contiguous(), w.to(dtype),
+                                   w.to(dtype), angle.cos(), angle.sin(), positions)]
+    odd = torch.zeros(M, D, dtype=torch.bool)
+    odd[torch.arange(M), at] = True
+    partner = at ^ 1 if interleaved else (at + rot // 2) % max(rot, 1)
+    turned = (at < rot) & (positions < P)
+    odd[torch.arange(M)[turned], partner[turned]] = True
+    for out, head in zip(K.qk_norm_rope(*args, EPS, interleaved), (1, 0)):
+        out = out.float().cpu()[0, :, head]
+        assert torch.equal(out.isnan(), odd) and not out[~odd].any()
+    dy = torch.randn(N, M, H, D, generator=g)
+    for m in range(0, M, max(1, M // 8)):  # one token at a time: one infinity
+        one = [t[:, m:m + 1] for t in args[:2]] + args[2:6] + [args[6][m:m + 1]]
+        dq = dy[:, m:m + 1].to(dtype).to(device)
+        grads = K.qk_norm_rope_grad(dq, dq[:, :, 1:].contiguous(), *one, EPS, interleaved)
+        alone = torch.arange(D) == at[m]
+        for dw in grads[2:]:
+            assert torch.equal(dw.cpu()[0].isnan(), alone)
+        # An infinite incoming gradient: the weights' gradient of its pair.
+        finite = [one[0][:, :, :1].contiguous(), one[1][:, :, 1:].contiguous(), *one[2:]]
+        dq[0, 0, 0, at[m]] = torch.inf
+        dq = dq[:, :, :1].contiguous()
+        grads = K.qk_norm_rope_grad(dq, dq, *finite, EPS, interleaved)
+        for dw in grads[2:]:
+            assert torch.equal(~dw.cpu()[0].isfinite(), odd[m])

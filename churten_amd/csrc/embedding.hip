@@ -809,6 +809,26 @@ int launch_direct(DirectArgs a, int64_t N, hipStream_t stream) {
 template <typename T, int G, bool NARROW>
 int launch_sorted(const GradPlan& p, SumArgs a, const ts_index& tokens, char* ws,
                   hipStream_t stream) {
+  constexpr int64_t kGroups = kThreads / G, kRows = kGroups * (G < 16 ? G : 16);
+  const int64_t zero_units = ceil_div(a.V, kRows);
+  const int64_t units = a.accumulate ? 0 : a.N * zero_units;
+  const auto zeros_before = [&](int merge) {  // of p.merges; without any: none
+    return p.merges > 0 ? units * merge / p.merges : 0;
+  };
+  a.chunks = p.chunks;
+  a.slices = p.slices;
+  a.chunk = p.chunk;
+  a.sum_blocks = ceil_div(p.chunks * p.slices, kGroups);
+  const auto merge_blocks = [&](int m) {
+    return p.lists * ceil_div(a.B, kThreads) + zeros_before(m + 1) - zeros_before(m);
+  };
+  const int64_t sum_blocks = a.N * a.sum_blocks + units - zeros_before(p.merges);
+  const int64_t joins = (p.chunks - 1) * p.slices;
+  // Before the first launch: a call that cannot end must not begin.
+  int64_t most = std::max(sum_blocks, joins);
+  for (int m = 0; m < p.merges; ++m) most = std::max(most, merge_blocks(m));
+  if (most > kMaxBlocks) return kInvalid;
+
   a.list_stride = p.lists == 1 ? 0 : a.B;
   // A list: all tokens, then all positions.
   auto* from = reinterpret_cast<int32_t*>(ws + p.list0);
@@ -850,7 +870,6 @@ int launch_sorted(const GradPlan& p, SumArgs a, const ts_index& tokens, char* ws
   }
   if (const int err = launched()) return err;
 
-  constexpr int64_t kGroups = kThreads / G, kRows = kGroups * (G < 16 ? G : 16);
   ZeroArgs zero{};
   zero.weight_grad = a.weight_grad;
   zero.tokens = tokens;
@@ -859,17 +878,14 @@ int launch_sorted(const GradPlan& p, SumArgs a, const ts_index& tokens, char* ws
   zero.B = a.B;
   zero.V = a.V;
   zero.D = a.D;
-  zero.units = ceil_div(a.V, kRows);
-  const int64_t units = a.accumulate ? 0 : a.N * zero.units;
+  zero.units = zero_units;
   int64_t runs = p.tiles;
   for (int m = 0; m < p.merges; ++m, runs = ceil_div(runs, kFan)) {
     const MergeArgs merge{from, from + half, to, to + half, p.lists, a.B,
                           p.tile_log2 + m * kFanLog2};
-    zero.first = units * m / p.merges;
-    zero.end = units * (m + 1) / p.merges;
-    const int64_t blocks = p.lists * ceil_div(a.B, kThreads) + zero.end - zero.first;
-    if (blocks > kMaxBlocks) return kInvalid;
-    const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
+    zero.first = zeros_before(m);
+    zero.end = zeros_before(m + 1);
+    const dim3 grid(static_cast<uint32_t>(merge_blocks(m))), block(kThreads);
     if (runs <= 4) {
       hipLaunchKernelGGL((merge_kernel<T, G, NARROW, 4>), grid, block, 0, stream, merge, zero);
     } else if (runs <= 8) {
@@ -881,23 +897,15 @@ int launch_sorted(const GradPlan& p, SumArgs a, const ts_index& tokens, char* ws
     if (const int err = launched()) return err;
     std::swap(from, to);
   }
-  zero.first = p.merges > 0 ? units : 0;
+  zero.first = zeros_before(p.merges);
   zero.end = units;
   a.token = from;
   a.position = from + half;
   a.parts = reinterpret_cast<float*>(ws + p.parts);
-  a.chunks = p.chunks;
-  a.slices = p.slices;
-  a.chunk = p.chunk;
-  a.sum_blocks = ceil_div(p.chunks * p.slices, kGroups);
-  const int64_t blocks = a.N * a.sum_blocks + zero.end - zero.first;
-  if (blocks > kMaxBlocks) return kInvalid;
-  hipLaunchKernelGGL((sum_kernel<T, G, NARROW>), dim3(static_cast<uint32_t>(blocks)),
+  hipLaunchKernelGGL((sum_kernel<T, G, NARROW>), dim3(static_cast<uint32_t>(sum_blocks)),
                      dim3(kThreads), 0, stream, a, zero);
   if (const int err = launched()) return err;
   if (p.chunks > 1) {
-    const int64_t joins = (p.chunks - 1) * p.slices;
-    if (joins > kMaxBlocks) return kInvalid;
     hipLaunchKernelGGL((join_kernel<T, G, NARROW>),
                        dim3(static_cast<uint32_t>(joins), static_cast<uint32_t>(a.N)),
                        dim3(kThreads), 0, stream, a);

@@ -372,3 +372,24 @@ def test_the_examples_gradients_are_those_of_plain_operations(device):
     for name, p in model.named_parameters():
         # float32 both ways; a dozen layers of operations on values near 1.
         torch.testing.assert_close(got[name], p.grad, rtol=2e-4, atol=2e-5)
+
+
+def test_a_gradient_too_large_for_its_launches_is_refused_before_any():
+    """No launch has 2^24 workgroups or more, and none is made of a call of which a
+    later one would: nothing is written, and without a GPU nothing else fails."""
+    lib = library()
+    most = 2 ** 31 - 2
+    rows = Rows(P, 1, 1)
+
+    def call(N, B, V, D, shared, flags=0):
+        size = lib.ts_embedding_grad_workspace(0, I64(N), I64(B), I64(V), I64(D), shared)
+        assert size > 0
+        index = Index(P, 0 if shared else B, 1, 64)
+        return lib.ts_embedding_grad(rows, rows, index, 0, I64(N), I64(B), I64(V), I64(D),
+                                     ctypes.c_float(1), flags, P, ctypes.c_size_t(size), None)
+
+    assert call(1, most, 100, 8, False) == 1  # joining its chunks
+    assert call(1, most, 100, 8, False, 1) == 1
+    assert call(16, 2 ** 29, 100, 8, False) == 1  # merging its lists
+    assert call(64, 300, most, 1, True) == 1  # zeroing its rows, without a merge
+    assert call(64, 9000, most, 1, True) == 1  # and beside one

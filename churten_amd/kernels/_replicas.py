@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 __all__ = ["OWN", "SHARED", "HYPER", "TABLE", "differentiable", "register_replica_vmap",
-           "without_derivative"]
+           "register_replica_vmap_", "without_derivative"]
 
 OWN = "own"  # every replica has one
 SHARED = "shared"  # the replicas may share one
@@ -71,6 +71,40 @@ def register_replica_vmap(name: str, kinds: list[tuple[str, int]], outputs: int)
         if replicas is not None:
             tensors = tuple(t.unflatten(0, (batch, replicas)) for t in tensors)
         return (tensors[0], 0) if outputs == 1 else (tensors, (0,) * outputs)
+
+    torch.library.register_vmap(f"churten::{name}", rule)
+
+
+def register_replica_vmap_(name: str, kinds: list[tuple[str, int]]) -> None:
+    """The same for an operator that writes into its first tensor and returns
+    nothing."""
+    op = getattr(torch.ops.churten, name)
+
+    def rule(info, in_dims, *args):
+        batch, dim = info.batch_size, in_dims[0]
+        if dim is None:
+            raise RuntimeError(f"churten::{name}: its first tensor is written in place, so "
+                               "vmap must be over it too")
+        out = args[0].movedim(dim, 0)
+        replicas = out.shape[1] if out.dim() - 1 > kinds[0][1] else None
+        given = list(args)
+        for i, (kind, rank) in enumerate(kinds[1:], 1):
+            given[i] = _fold(given[i], in_dims[i], kind, rank, batch, replicas)
+        if replicas is None:
+            op(out, *given[1:])
+            return None, None
+        try:
+            folded = out.view(batch * replicas, *out.shape[2:])
+        except RuntimeError:  # no one view: a call for each
+            folded = None
+        if folded is not None:
+            op(folded, *given[1:])
+            return None, None
+        for b in range(batch):
+            own = slice(b * replicas, (b + 1) * replicas)
+            op(out[b], *(t[own] if i < len(kinds) and t.dim() > kinds[i][1] else t
+                         for i, t in enumerate(given[1:], 1)))
+        return None, None
 
     torch.library.register_vmap(f"churten::{name}", rule)
 

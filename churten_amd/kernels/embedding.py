@@ -29,6 +29,7 @@ from churten_amd.kernels._replicas import (
     SHARED,
     differentiable,
     register_replica_vmap,
+    register_replica_vmap_,
 )
 
 embedding_grad = torch.ops.churten.embedding_grad
@@ -91,3 +92,4 @@ def embedding(weight: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0) ->
 
 register_replica_vmap("embedding", [(OWN, 2), (SHARED, 1)], outputs=1)
 register_replica_vmap("embedding_grad", [(OWN, 2), (SHARED, 1)], outputs=1)
+register_replica_vmap_("embedding_grad_", [(OWN, 2), (OWN, 2), (SHARED, 1)])

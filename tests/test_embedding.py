@@ -341,3 +341,42 @@ def test_tables_of_more_than_2_to_the_31_elements(device):
         assert (weight[0, -1] == B // 2).all() and (weight[0, 65535] == B // 4).all()
         assert (weight[0, 0] == B // 4).all() and not weight[0, 1:65535].any()
         assert not weight[0, 65536:-1].any()
+
+
+def test_gradient_in_place_under_vmap(device):
+    """Over one replica's code, over calls with replicas, and along a dimension that
+    is not the first; what the replicas share is shared."""
+    g = gen(15)
+    S, N, B, V, D = 4, 3, 70, 11, 6
+    grad = torch.randn(S, N, B, D, generator=g).to(device)
+    tokens = torch.randint(-1, V, (S, N, B), generator=g).to(device)
+    before = torch.randn(S, N, V, D, generator=g).to(device)
+    want = torch.stack([K.embedding_grad(grad[s], tokens[s], V, 0.5) for s in range(S)])
+
+    def write(out, grad, tokens, scale=0.5, accumulate=False):
+        K.embedding_grad_(out, grad, tokens, scale, accumulate=accumulate)
+        return out
+
+    flat = torch.zeros(N, 3 + V * D, device=device)
+    view = flat[:, 3:].view(N, V, D)
+    vmap(write)(view, grad[0], tokens[0])
+    assert torch.equal(view, want[0]) and not flat[:, :3].any()
+    out = before.clone()
+    vmap(lambda o, g, t: write(o, g, t, accumulate=True))(out, grad, tokens)
+    each = before.clone()
+    for s in range(S):
+        K.embedding_grad_(each[s], grad[s], tokens[s], 0.5, accumulate=True)
+    assert torch.equal(out, each)
+    # Rows of all of them that no one view holds: (N, S, V, D) of a wider buffer.
+    wide = torch.zeros(N, S, V, 2 * D, device=device)
+    vmap(write, in_dims=(1, 0, 0))(wide[..., :D], grad, tokens)
+    assert torch.equal(wide[..., :D].transpose(0, 1), want) and not wide[..., D:].any()
+    # Twice, with shared tokens and a shared gradient.
+    out = torch.zeros(S, N, V, D, device=device)
+    vmap(vmap(lambda o: write(o, grad[0, 0], tokens[0, 0], 1.0)))(out)
+    assert torch.equal(out, K.embedding_grad(grad[0, 0], tokens[0, 0], V).expand(S, N, V, D))
+    out = torch.zeros(S, N, V, D, device=device)
+    vmap(lambda o, g: write(o, g, tokens[0], 1.0))(out, grad)
+    assert torch.equal(out[2], K.embedding_grad(grad[2], tokens[0], V))
+    with pytest.raises(RuntimeError, match="written in place"):
+        vmap(lambda g: write(out[0], g, tokens[0]))(grad)

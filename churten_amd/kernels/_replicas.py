@@ -4,10 +4,13 @@
 straight to the operator; the others through a ``torch.autograd.Function``,
 which plain autograd and the transforms of ``torch.func`` both take.
 
-``register_replica_vmap`` is the operators' batching rule. They take their tensors with a leading replica dimension, or all of them
-without, and some may be shared by the replicas. So an outer
+``register_replica_vmap`` is the operators' batching rule. They take their
+tensors with a leading replica dimension, or all of them without, and some may
+be shared by the replicas. So an outer
 ``torch.func.vmap`` dimension is a replica dimension: over a call without one
-it becomes it, over a call that has one both are folded together.
+it becomes it, over a call that has one both are folded together -- where a
+replica's own tensor that vmap is not over is repeated in memory, once for each
+of the batch (but for the table of a lookup).
 """
 
 from __future__ import annotations
@@ -15,7 +18,7 @@ from __future__ import annotations
 import torch
 
 __all__ = ["OWN", "SHARED", "HYPER", "TABLE", "differentiable", "register_replica_vmap",
-           "register_replica_vmap_", "without_derivative"]
+           "register_replica_vmap_", "replica_vmap", "without_derivative"]
 
 OWN = "own"  # every replica has one
 SHARED = "shared"  # the replicas may share one
@@ -44,8 +47,8 @@ def _fold(t, dim, kind, rank, batch, replicas):
     return t.expand(batch, replicas, *t.shape[2:]).flatten(0, 1)
 
 
-def register_replica_vmap(name: str, kinds: list[tuple[str, int]], outputs: int) -> None:
-    """``kinds``: for each tensor argument, in order, what it is to a replica
+def replica_vmap(name: str, kinds: list[tuple[str, int]], outputs: int):
+    """The batching rule of ``churten::name``. ``kinds``: for each tensor argument, in order, what it is to a replica
     and its dimensions for one; the first is a replica's own and shows whether
     the call has the replicas' dimension. ``outputs``: how many tensors the
     operator returns."""
@@ -72,7 +75,11 @@ def register_replica_vmap(name: str, kinds: list[tuple[str, int]], outputs: int)
             tensors = tuple(t.unflatten(0, (batch, replicas)) for t in tensors)
         return (tensors[0], 0) if outputs == 1 else (tensors, (0,) * outputs)
 
-    torch.library.register_vmap(f"churten::{name}", rule)
+    return rule
+
+
+def register_replica_vmap(name: str, kinds: list[tuple[str, int]], outputs: int) -> None:
+    torch.library.register_vmap(f"churten::{name}", replica_vmap(name, kinds, outputs))
 
 
 def register_replica_vmap_(name: str, kinds: list[tuple[str, int]]) -> None:

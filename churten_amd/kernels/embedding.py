@@ -30,6 +30,7 @@ from churten_amd.kernels._replicas import (
     differentiable,
     register_replica_vmap,
     register_replica_vmap_,
+    replica_vmap,
 )
 
 embedding_grad = torch.ops.churten.embedding_grad
@@ -90,6 +91,17 @@ def embedding(weight: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0) ->
     return _apply(weight, tokens, scale)
 
 
-register_replica_vmap("embedding", [(OWN, 2), (SHARED, 1)], outputs=1)
+def _lookups(info, in_dims, weight, tokens, scale=1.0):
+    """A table that vmap is not over is looked up once, by the tokens of the whole
+    batch: folding the batch into its replicas would repeat it."""
+    if in_dims[0] is not None:
+        return _replica_lookups(info, in_dims, weight, tokens, scale)
+    tokens = tokens.movedim(in_dims[1], -2)
+    out = _op(weight, tokens.flatten(-2), scale).unflatten(-2, tokens.shape[-2:])
+    return out, out.dim() - 3
+
+
+_replica_lookups = replica_vmap("embedding", [(OWN, 2), (SHARED, 1)], outputs=1)
+torch.library.register_vmap("churten::embedding", _lookups)
 register_replica_vmap("embedding_grad", [(OWN, 2), (SHARED, 1)], outputs=1)
 register_replica_vmap_("embedding_grad_", [(OWN, 2), (OWN, 2), (SHARED, 1)])

@@ -380,3 +380,37 @@ def test_gradient_in_place_under_vmap(device):
     assert torch.equal(out[2], K.embedding_grad(grad[2], tokens[0], V))
     with pytest.raises(RuntimeError, match="written in place"):
         vmap(lambda g: write(out[0], g, tokens[0]))(grad)
+
+
+def test_a_table_that_vmap_is_not_over_is_not_repeated(device):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Largest(TorchDispatchMode):
+        bytes = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (tuple, list)) else (out,):
+                if isinstance(t, torch.Tensor) and t.untyped_storage().data_ptr() not in known:
+                    self.bytes = max(self.bytes, t.untyped_storage().nbytes())
+            return out
+
+    g = gen(16)
+    S, N, B, V, D = 5, 3, 4, 2000, 8
+    weight = torch.randn(N, V, D, generator=g).to(device)
+    tokens = torch.randint(-1, V + 1, (S, N, B), generator=g).to(device)
+    known = {weight.untyped_storage().data_ptr()}
+    want = torch.stack([K.embedding(weight, ids, 0.5) for ids in tokens])
+    for w, ids, dim, expected in ((weight, tokens, 0, want),
+                                  (weight, tokens.movedim(0, 2), 2, want),
+                                  (weight, tokens[:, 0], 0, torch.stack(
+                                      [K.embedding(weight, ids, 0.5) for ids in tokens[:, 0]])),
+                                  (weight[0], tokens[:, 0], 0, want[:, 0])):
+        with Largest() as largest:
+            got = vmap(lambda t: K.embedding(w, t, 0.5), in_dims=dim)(ids)
+        assert torch.equal(got, expected)
+        assert largest.bytes < N * V * D * 4
+    # Its gradient adds up over the batch.
+    up = torch.randint(-3, 4, (S, N, B, D), generator=g).float().to(device)
+    got = func_grad(lambda w: (vmap(lambda t: K.embedding(w, t, 2.0))(tokens) * up).sum())(weight)
+    assert torch.equal(got, sum(K.embedding_grad(u, t, V, 2.0) for u, t in zip(up, tokens)))

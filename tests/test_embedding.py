@@ -414,3 +414,28 @@ def test_a_table_that_vmap_is_not_over_is_not_repeated(device):
     up = torch.randint(-3, 4, (S, N, B, D), generator=g).float().to(device)
     got = func_grad(lambda w: (vmap(lambda t: K.embedding(w, t, 2.0))(tokens) * up).sum())(weight)
     assert torch.equal(got, sum(K.embedding_grad(u, t, V, 2.0) for u, t in zip(up, tokens)))
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("kind", ["zipf", "one", "outside", "even"])
+@pytest.mark.parametrize("B", [12289, 16384, 16385, 20000, 32768, 32769, 65536])
+def test_gradient_of_lists_of_four_to_sixteen_tiles(device, B, kind, shared):
+    """One merge of up to four, eight and sixteen runs, the last of them whole or short."""
+    g = gen(17)
+    V, D = 5000, 4
+    grad = torch.randn(2, B, D, generator=g)
+    tokens = make_tokens(kind, 1 if shared else 2, B, V, g)
+    want, bound = embedding_grad(grad, tokens.expand(2, B), V, 0.7)
+    given = tokens[0] if shared else tokens
+    assert_within(K.embedding_grad(grad.to(device), given.to(device), V, 0.7), want, bound)
+
+
+@pytest.mark.parametrize("B", [20000, 40000])
+def test_gradient_of_many_tiles_of_a_very_large_vocabulary(device, B):
+    """Sorted words of 64 bits, merged."""
+    g = gen(18)
+    V, D = 2 ** 21, 2
+    grad = torch.randn(1, B, D, generator=g)
+    tokens = make_tokens("zipf", 1, B, V, g)
+    want, bound = embedding_grad(grad, tokens, V, 1.0)
+    assert_within(K.embedding_grad(grad.to(device), tokens.to(device), V), want, bound)

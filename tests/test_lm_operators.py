@@ -393,3 +393,41 @@ def test_a_gradient_too_large_for_its_launches_is_refused_before_any():
     assert call(16, 2 ** 29, 100, 8, False) == 1  # merging its lists
     assert call(64, 300, most, 1, True) == 1  # zeroing its rows, without a merge
     assert call(64, 9000, most, 1, True) == 1  # and beside one
+
+
+@pytest.mark.gpu
+def test_graph_replays_follow_the_tokens():
+    """Every launch sequence of the embedding, with other tokens, tables and
+    incoming gradients at each replay."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    V = 3000
+    calls = []
+    for B in (90, 900, 5000, 20000, 40000, 70000):
+        for lead in ((2,), ()):  # a list for each replica, and one for both
+            tokens = torch.randint(-1, V + 1, (*lead, B), generator=g, device="cuda")
+            grad = torch.randn(2, B, 6, generator=g, device="cuda")
+            into = torch.zeros(2, V, 6, device="cuda")
+            calls.append((K.embedding_grad, [grad, tokens, V]))
+            calls.append((lambda o, g, t: K.embedding_grad_(o, g, t) or o, [into, grad, tokens]))
+    calls.append((K.embedding, [torch.randn(2, V, 6, device="cuda"), tokens]))
+    for call, args in calls:
+        call(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [call(*args) for call, args in calls]
+    for turn in range(4):
+        for call, args in calls:
+            for t in args:
+                if isinstance(t, torch.Tensor) and t.is_floating_point():
+                    t.normal_()
+                elif isinstance(t, torch.Tensor):
+                    t.random_(-1, (V, 20, V + 5, 1)[turn])
+        eager = [call(*args).clone() for call, args in calls]
+        for _, args in calls:
+            if len(args) == 3 and isinstance(args[2], torch.Tensor):
+                args[0].fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for want, got in zip(eager, held):
+            assert torch.equal(want, got), turn

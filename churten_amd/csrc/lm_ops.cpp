@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
@@ -500,11 +501,12 @@ void implement(Library& m) {
 // ---------------------------------------------------------------------------
 // Derivatives
 // ---------------------------------------------------------------------------
-// The operators themselves have none -- those of the forward ones are formed a
-// level above, in Python -- and asking for one, in reverse or in forward mode,
+// Asking for a derivative that is not there, in reverse or in forward mode,
 // raises (torch's default for an operator of a library is a warning, zeros, and
-// a tangent that is dropped). torch's own kernel for that goes through every
-// argument in its boxed form, 0.2 us of a lookup's 2.2 us on the host; this one 0.05.
+// a tangent that is dropped). The heads and the distillation have none at this
+// level: those of the forward operators are formed a level above, in Python.
+// torch's own kernel for that goes through every argument in its boxed form, 0.2
+// us of a lookup's 2.2 us on the host; this one 0.05.
 bool needs_derivative(const at::Tensor& t) { return t.requires_grad(); }
 bool needs_derivative(const std::optional<at::Tensor>& t) {
   return t.has_value() && t->requires_grad();
@@ -563,21 +565,92 @@ struct Underived<R(A...)> {
   static void add(torch::autograd::edge_list&, double) {}
 };
 
-// In place, as torch's own: a target that gradients would go through is refused or
-// remembers that they cannot, and its version counter rises.
+template <typename Function>
+auto operator_of(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Function>();
+}
+const auto& embedding_op() {
+  static const auto op = operator_of<decltype(embedding)>("churten::embedding");
+  return op;
+}
 const auto& embedding_grad_op() {
-  static const auto op = c10::Dispatcher::singleton()
-                             .findSchemaOrThrow("churten::embedding_grad_", "")
-                             .typed<decltype(embedding_grad_)>();
+  static const auto op = operator_of<decltype(embedding_grad)>("churten::embedding_grad");
+  return op;
+}
+const auto& embedding_grad_into_op() {
+  static const auto op = operator_of<decltype(embedding_grad_)>("churten::embedding_grad_");
   return op;
 }
 
+void refuse_tangent(const char* op, const at::Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), op, " has no derivative in forward AD mode");
+}
+
+// The lookup is linear in the table and its gradient in the incoming one; each is
+// the other's derivative, so both have derivatives of every order.
+struct LookupDerivative : torch::autograd::Node {
+  torch::autograd::SavedVariable tokens;
+  int64_t num_embeddings = 0;
+  double scale = 1;
+  bool of_gradient = false;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const at::Tensor& grad = grads[0];
+    if (!grad.defined()) return {at::Tensor()};
+    const at::Tensor ids = tokens.unpack();
+    return {of_gradient ? embedding_op().call(grad, ids, scale)
+                        : embedding_grad_op().call(grad, ids, num_embeddings, scale)};
+  }
+  void release_variables() override { tokens.reset_data(); }
+};
+
+// `out` with the derivative in `in`, if that asks for one.
+at::Tensor derived(const at::Tensor& in, const at::Tensor& tokens, at::Tensor out,
+                   int64_t num_embeddings, double scale, bool of_gradient) {
+  if (!at::GradMode::is_enabled() || !in.requires_grad()) return out;
+  const std::shared_ptr<LookupDerivative> node(new LookupDerivative,
+                                               torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(in));
+  node->tokens = torch::autograd::SavedVariable(tokens, /*is_output=*/false);
+  node->num_embeddings = num_embeddings;
+  node->scale = scale;
+  node->of_gradient = of_gradient;
+  torch::autograd::set_history(out, node);
+  return out;
+}
+
+at::Tensor embedding_derived(c10::DispatchKeySet keys, const at::Tensor& weight,
+                             const at::Tensor& tokens, double scale) {
+  refuse_tangent("churten::embedding", weight);
+  at::Tensor out = [&] {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return embedding_op().redispatch(keys & c10::after_autograd_keyset, weight, tokens, scale);
+  }();
+  // Traced with sizes as symbols, the table's is made a number.
+  const int64_t V = weight.sym_size(-2).guard_int(__FILE__, __LINE__);
+  return derived(weight, tokens, std::move(out), V, scale, false);
+}
+
+at::Tensor embedding_grad_derived(c10::DispatchKeySet keys, const at::Tensor& grad,
+                                  const at::Tensor& tokens, int64_t num_embeddings,
+                                  double scale) {
+  refuse_tangent("churten::embedding_grad", grad);
+  at::Tensor out = [&] {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return embedding_grad_op().redispatch(keys & c10::after_autograd_keyset, grad, tokens,
+                                          num_embeddings, scale);
+  }();
+  return derived(grad, tokens, std::move(out), num_embeddings, scale, true);
+}
+
+// In place, as torch's own: a target that gradients would go through is refused or
+// remembers that they cannot, and its version counter rises.
 void embedding_grad_underived(c10::DispatchKeySet keys, at::Tensor weight_grad,
                               const at::Tensor& grad, const at::Tensor& tokens, double scale,
                               bool accumulate) {
   constexpr const char* op = "churten::embedding_grad_";
-  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(weight_grad) && !has_tangent(grad), op,
-                              " has no derivative in forward AD mode");
+  refuse_tangent(op, weight_grad);
+  refuse_tangent(op, grad);
   const bool any = at::GradMode::is_enabled() &&
                    (needs_derivative(weight_grad) || needs_derivative(grad));
   torch::autograd::check_inplace(weight_grad, any);
@@ -590,8 +663,8 @@ void embedding_grad_underived(c10::DispatchKeySet keys, at::Tensor weight_grad,
   }
   {
     const at::AutoDispatchBelowAutograd below;
-    embedding_grad_op().redispatch(keys & c10::after_autograd_keyset, weight_grad, grad, tokens,
-                                   scale, accumulate);
+    embedding_grad_into_op().redispatch(keys & c10::after_autograd_keyset, weight_grad, grad,
+                                        tokens, scale, accumulate);
   }
   if (any) torch::autograd::rebase_history(weight_grad, node);
 }
@@ -601,10 +674,11 @@ void embedding_grad_written(c10::DispatchKeySet keys, at::Tensor weight_grad,
                             bool accumulate) {
   {
     const at::AutoDispatchBelowADInplaceOrView below;
-    embedding_grad_op().redispatch(keys & c10::after_ADInplaceOrView_keyset, weight_grad, grad,
-                                   tokens, scale, accumulate);
+    embedding_grad_into_op().redispatch(keys & c10::after_ADInplaceOrView_keyset, weight_grad,
+                                        grad, tokens, scale, accumulate);
   }
-  torch::autograd::increment_version(weight_grad);
+  // One made in inference mode has no counter.
+  if (!weight_grad.is_inference()) torch::autograd::increment_version(weight_grad);
 }
 
 }  // namespace
@@ -633,8 +707,6 @@ TORCH_LIBRARY_IMPL(churten, CUDA, m) { implement(m); }
 TORCH_LIBRARY_IMPL(churten, CPU, m) { implement(m); }
 
 namespace {
-constexpr char kEmbedding[] = "churten::embedding";
-constexpr char kEmbeddingGrad[] = "churten::embedding_grad";
 constexpr char kQkNormRope[] = "churten::qk_norm_rope";
 constexpr char kQkNormRopeGrad[] = "churten::qk_norm_rope_grad";
 constexpr char kDistillLoss[] = "churten::distill_loss";
@@ -642,8 +714,8 @@ constexpr char kDistillLossGrad[] = "churten::distill_loss_grad";
 }  // namespace
 
 TORCH_LIBRARY_IMPL(churten, Autograd, m) {
-  m.impl("embedding", &Underived<decltype(embedding)>::call<kEmbedding>);
-  m.impl("embedding_grad", &Underived<decltype(embedding_grad)>::call<kEmbeddingGrad>);
+  m.impl("embedding", &embedding_derived);
+  m.impl("embedding_grad", &embedding_grad_derived);
   m.impl("embedding_grad_", &embedding_grad_underived);
   m.impl("qk_norm_rope", &Underived<decltype(qk_norm_rope)>::call<kQkNormRope>);
   m.impl("qk_norm_rope_grad", &Underived<decltype(qk_norm_rope_grad)>::call<kQkNormRopeGrad>);

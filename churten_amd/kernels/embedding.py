@@ -15,8 +15,8 @@
   another layer shares), where rows that no token names are not touched.
 
 All of them without the replica dimension are one replica's call. ``embedding``
-is differentiable in ``weight``, as often as asked for, and composes with
-``torch.func.vmap``; a derivative of ``embedding_grad`` itself raises.
+is differentiable in ``weight`` and ``embedding_grad`` in ``grad``, as often as
+asked for in reverse mode; all compose with ``torch.func.vmap``.
 """
 
 from __future__ import annotations
@@ -27,12 +27,12 @@ from churten_amd.kernels import _C  # noqa: F401  (registers the ops)
 from churten_amd.kernels._replicas import (
     OWN,
     SHARED,
-    differentiable,
     register_replica_vmap,
     register_replica_vmap_,
     replica_vmap,
 )
 
+_op = torch.ops.churten.embedding.default
 embedding_grad = torch.ops.churten.embedding_grad
 embedding_grad_ = torch.ops.churten.embedding_grad_
 
@@ -54,41 +54,9 @@ def _embedding_grad_into_fake(weight_grad, grad, tokens, scale=1.0, accumulate=F
     return None
 
 
-def _setup(ctx, inputs, output):
-    weight, tokens, ctx.scale = inputs
-    ctx.num_embeddings = weight.shape[-2]
-    ctx.save_for_backward(tokens)
-
-
-def _backward(ctx, grad):
-    tokens, = ctx.saved_tensors
-    # A compiled backward pass is not differentiated again.
-    once = torch.compiler.is_compiling() or (
-        _plain() and not (grad.requires_grad and torch.is_grad_enabled()))
-    form = embedding_grad if once else _grad_apply
-    return form(grad, tokens, ctx.num_embeddings, ctx.scale), None, None
-
-
-def _grad_setup(ctx, inputs, output):
-    _, tokens, _, ctx.scale = inputs
-    ctx.save_for_backward(tokens)
-
-
-def _grad_backward(ctx, grad):
-    # The gradient is linear in the incoming one; its transpose is the lookup.
-    tokens, = ctx.saved_tensors
-    return embedding(grad, tokens, ctx.scale), None, None, None
-
-
-_, _grad_apply, _ = differentiable("embedding_grad", _grad_setup, _grad_backward)
-_op, _apply, _plain = differentiable("embedding", _setup, _backward)
-
-
 def embedding(weight: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``scale * weight[n, tokens[n, b]]``; see the module's description."""
-    if _plain() and not (weight.requires_grad and torch.is_grad_enabled()):
-        return _op(weight, tokens, scale)
-    return _apply(weight, tokens, scale)
+    return _op(weight, tokens, scale)
 
 
 def _lookups(info, in_dims, weight, tokens, scale=1.0):

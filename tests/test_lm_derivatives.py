@@ -97,16 +97,22 @@ def test_a_second_derivative_that_is_not_there_raises(device):
 
 
 def test_a_derivative_of_a_gradient_operator_raises(device):
-    _, tokens = table(device)
-    grad = torch.ones(2, 9, 5, device=device, requires_grad=True)
     row = rows(device)
     row[0].requires_grad_()
     q, k, *rest = heads(device)
     q.requires_grad_()
-    for out in (K.embedding_grad(grad, tokens, 7), K.distill_loss_grad(*row)[0],
+    for out in (K.distill_loss_grad(*row)[0],
                 K.qk_norm_rope_grad(torch.ones_like(q), torch.ones_like(k), q, k, *rest)[2]):
         with pytest.raises(RuntimeError, match="not implemented"):
             out.sum().backward()
+
+
+def test_the_embedding_gradient_is_differentiable(device):
+    _, tokens = table(device)
+    grad = torch.ones(2, 9, 5, device=device, requires_grad=True)
+    up = torch.arange(70.0, device=device).view(2, 7, 5)
+    (K.embedding_grad(grad, tokens, 7, 2.0) * up).sum().backward()
+    assert torch.equal(grad.grad, K.embedding(up, tokens, 2.0))
 
 
 def test_forward_mode_raises(device):
@@ -206,3 +212,26 @@ def test_no_gradient_flows_to_the_teacher(device):
     assert torch.equal(leaf.grad, K.distill_loss_grad(x, z, index, t)[1])
     both = func_grad(lambda x, z: K.distill_loss(x, z, index, t).sum(), argnums=(0, 1))(x, z)
     assert torch.equal(both[0], leaf.grad) and not both[1].any()
+
+
+def test_embedding_in_inference_mode_and_traced_with_symbols(device):
+    weight, tokens = table(device)
+    grad = torch.ones(2, 9, 5, device=device)
+    want = K.embedding_grad(grad, tokens, 7)
+    with torch.inference_mode():
+        made = torch.zeros(2, 7, 5, device=device)
+        assert torch.equal(K.embedding(weight, tokens, 2.0), lookups(tokens)[1](weight))
+    K.embedding_grad_(made, grad, tokens)
+    assert torch.equal(made, want)
+    with torch.inference_mode():
+        K.embedding_grad_(made, grad, tokens, accumulate=True)
+    assert torch.equal(made, 2 * want)
+
+    def loss(w, ids):
+        return (K.embedding(w, ids, 2.0) ** 2).sum()
+
+    compiled = torch.compile(loss, backend="aot_eager", dynamic=True, fullgraph=True)
+    for V, B in ((7, 9), (6, 5), (4, 8)):
+        leaf, ids = weight[:, :V].clone().requires_grad_(), tokens[:, :B] % V
+        got, = torch.autograd.grad(compiled(leaf, ids), leaf)
+        assert torch.equal(got, torch.autograd.grad(loss(leaf, ids), leaf)[0])
